@@ -464,35 +464,8 @@ static uint32_t find_best_partition_order(enc_ws *w, const int32_t *res, uint32_
 }
 
 /* ------------------------------------------------------------------ fixed predictor */
-/* The reference binary (x86-64, AVX2 dispatch) computes the error sums of the "wide" and "limit_residual" variants with
- * FLAC__fixed_compute_best_predictor_wide_intrin_avx2 / _limit_residual_intrin_avx2: four lanes walk data_len/4 samples
- * each.  The lanes' histories are taken at j*(data_len/4), but the lanes START at data_len/4, (2*data_len)/4 and
- * (3*data_len)/4; the data_len%4 samples behind the lanes are ignored by the _wide routine and added by a scalar loop in
- * the _limit_residual routine.  When data_len is a multiple of four this
- * is the exact sum; otherwise lanes 2 and 3 start one or two samples late against their history and the sums differ
- * from the plain C loop (which the same library uses on CPUs without AVX2).  Recovered from the disassembly of the
- * reference binary and pinned by tests/tools/fuzz_oracle_vs_ref.py; sums are what pyFLAC users on x86-64 get. */
-static void avx2_lane_sums(const int64_t *d, uint32_t len, uint64_t t[5], int over[5])
-{
-    const uint32_t q = len / 4;
-    const uint32_t start[4] = {0, len >> 2, len >> 1, (3 * len) >> 2};
-    if (len < 4) return;
-    for (int j = 0; j < 4; j++) {
-        const int64_t *h = d + (size_t)j * q;
-        int64_t p0 = h[-1], p1 = h[-1] - h[-2], p2 = p1 - (h[-2] - h[-3]), p3 = p2 - (h[-2] - 2 * h[-3] + h[-4]);
-        for (uint32_t i = 0; i < q; i++) {
-            const int64_t e0 = d[start[j] + i], e1 = e0 - p0, e2 = e1 - p1, e3 = e2 - p2, e4 = e3 - p3;
-            const int64_t e[5] = {e0, e1, e2, e3, e4};
-            for (int k = 0; k < 5; k++) {
-                const uint64_t a = (uint64_t)(e[k] < 0 ? -e[k] : e[k]);
-                t[k] += a;
-                if (a > 0x7FFFFFFF) over[k] = 1;
-            }
-            p3 = e3; p2 = e2; p1 = e1; p0 = e0;
-        }
-    }
-}
-
+/* The error sums are plain: every sample from the fifth on counts once, for every sample width and block length (the four
+ * warm-up positions as well where an order's residual has to fit 32 bits, from 28 bits a sample on). */
 static uint32_t fixed_best_predictor(const int64_t *x, uint32_t n, uint32_t sbps, float rbps[5], uint64_t tot[5])
 {
     /* x points at the start of the block */
@@ -501,21 +474,12 @@ static uint32_t fixed_best_predictor(const int64_t *x, uint32_t n, uint32_t sbps
         uint64_t t0 = 0, t1 = 0, t2 = 0, t3 = 0, t4 = 0;
         const int64_t *d = x + 4;
         const uint32_t len = n - 4;
-        /* stream_encoder.c process_subframe_: 32-bit accumulators while sbps + ilog2((blocksize-4)*17) < 32, else _wide */
-        if (sbps + ilog2_32(len * 17) < 32) {
-            for (int i = 0; i < (int)len; i++) {
-                int32_t e0 = (int32_t)d[i], e1 = (int32_t)(d[i] - d[i - 1]), e2 = (int32_t)(d[i] - 2 * d[i - 1] + d[i - 2]);
-                int32_t e3 = (int32_t)(d[i] - 3 * d[i - 1] + 3 * d[i - 2] - d[i - 3]);
-                int32_t e4 = (int32_t)(d[i] - 4 * d[i - 1] + 6 * d[i - 2] - 4 * d[i - 3] + d[i - 4]);
-                t0 += (uint32_t)abs(e0); t1 += (uint32_t)abs(e1); t2 += (uint32_t)abs(e2);
-                t3 += (uint32_t)abs(e3); t4 += (uint32_t)abs(e4);
-            }
-        }
-        else {
-            uint64_t t[5] = {0, 0, 0, 0, 0};
-            int over[5] = {0, 0, 0, 0, 0};
-            avx2_lane_sums(d, len, t, over);
-            t0 = t[0]; t1 = t[1]; t2 = t[2]; t3 = t[3]; t4 = t[4];
+        for (int i = 0; i < (int)len; i++) {
+            int32_t e0 = (int32_t)d[i], e1 = (int32_t)(d[i] - d[i - 1]), e2 = (int32_t)(d[i] - 2 * d[i - 1] + d[i - 2]);
+            int32_t e3 = (int32_t)(d[i] - 3 * d[i - 1] + 3 * d[i - 2] - d[i - 3]);
+            int32_t e4 = (int32_t)(d[i] - 4 * d[i - 1] + 6 * d[i - 2] - 4 * d[i - 3] + d[i - 4]);
+            t0 += (uint32_t)abs(e0); t1 += (uint32_t)abs(e1); t2 += (uint32_t)abs(e2);
+            t3 += (uint32_t)abs(e3); t4 += (uint32_t)abs(e4);
         }
         tot[0] = t0; tot[1] = t1; tot[2] = t2; tot[3] = t3; tot[4] = t4;
 #define MIN2(a, b) ((a) < (b) ? (a) : (b))
@@ -528,18 +492,14 @@ static uint32_t fixed_best_predictor(const int64_t *x, uint32_t n, uint32_t sbps
             rbps[k] = (float)((tot[k] > 0) ? log(M_LN2 * (double)tot[k] / (double)len) / M_LN2 : 0.0);
     }
     else {
-        /* _limit_residual variants: the sums include the four warm-up positions (i = -4..-1), and an order whose
-         * residual would not fit int32 is disqualified.  sbps <= 32: the AVX2 lanes above; sbps == 33 (side channel
-         * of a 32-bit stream): FLAC__fixed_compute_best_predictor_limit_residual_33bit, plain C, every sample. */
+        /* _limit_residual rules: the sums include the four warm-up positions (i = -4..-1), and an order whose
+         * residual would not fit int32 is disqualified. */
         uint64_t t[5] = {0, 0, 0, 0, 0}, smallest = UINT64_MAX;
         int over[5] = {0, 0, 0, 0, 0};
         const int64_t *d = x + 4;
         const uint32_t len = n - 4;
         for (int i = -4; i < (int)len; i++) {
             uint64_t e[5];
-            /* sbps <= 32: the scalar parts of the AVX2 routine are the warm-up positions and the len%4 samples at the
-             * end (which the shifted lanes may already have counted once) */
-            if (sbps <= 32 && i >= 0 && i < (int)(len & ~3u)) continue;
             e[0] = (uint64_t)llabs((long long)d[i]);
             e[1] = (i > -4) ? (uint64_t)llabs((long long)d[i] - d[i - 1]) : 0;
             e[2] = (i > -3) ? (uint64_t)llabs((long long)d[i] - 2 * (long long)d[i - 1] + d[i - 2]) : 0;
@@ -547,7 +507,6 @@ static uint32_t fixed_best_predictor(const int64_t *x, uint32_t n, uint32_t sbps
             e[4] = (i > -1) ? (uint64_t)llabs((long long)d[i] - 4 * (long long)d[i - 1] + 6 * (long long)d[i - 2] - 4 * (long long)d[i - 3] + d[i - 4]) : 0;
             for (int k = 0; k < 5; k++) { t[k] += e[k]; if (e[k] > 0x7FFFFFFF) over[k] = 1; }
         }
-        if (sbps <= 32) avx2_lane_sums(d, len, t, over);
         /* Observed on the reference binary (true 32-bit probes, tests/test_oracle_vs_reference.py):
          * ties go to the lowest order, a non-zero constant signal is NOT flagged constant and an
          * all-zero one is; i.e. the per-order estimate is derived from total_error_0 for every order. */

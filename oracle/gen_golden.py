@@ -64,7 +64,7 @@ def main():
                      'frame_bytes': [len(c[0]) for c in cbs[3:]], 'pcm_hash': synth.pcm_hash(arr)}
         print('%-24s %8d bytes  %s' % (name, len(stream), lim[name]['sha256'][:16]))
     # seeded random corpus (tests/fuzzgen.py): settings, sample formats and signal families well outside the named cases,
-    # incl. 32-bit stereo (33-bit side channel) and ragged blocks above 16 bit (the binary's AVX2 fixed-predictor sums)
+    # incl. 32-bit stereo (33-bit side channel) and ragged blocks above 16 bit 
     from tests import fuzzgen
     fz = {}
     for seed in range(fuzzgen.GOLDEN_SEEDS):

@@ -244,51 +244,22 @@ struct Enc {
     }
 
     // ---------------------------------------------------------------- fixed predictor sums (L4)
-    // Error sums the way the reference binary's AVX2 routines take them (oracle/flac_oracle.c avx2_lane_sums): four lanes
-    // of len/4 samples whose histories sit at j*(len/4) while the lanes start at (j*len)/4.  Only called when len is not a
-    // multiple of four (otherwise this is the plain sum).  d(i) = sample 4+i of the block.
-    __device__ void lane_sums(int c, uint32_t w, uint32_t len, u64 a[5], uint32_t *inv)
-    {
-        const uint32_t q = len >> 2;
-        for (uint32_t idx = lane; idx < 4 * q; idx += 64) {
-            const uint32_t j = idx / q, i = idx - j * q;
-            const uint32_t hb = 4 + j * q, st = 4 + ((j * len) >> 2);
-            i64 v[5];
-            for (uint32_t m = 0; m < 5; m++) v[m] = i >= m ? get64(c, st + i - m, w) : get64(c, hb + i - m, w);
-            const i64 e[5] = {v[0], v[0] - v[1], v[0] - 2 * v[1] + v[2], v[0] - 3 * v[1] + 3 * v[2] - v[3],
-                              v[0] - 4 * v[1] + 6 * v[2] - 4 * v[3] + v[4]};
-            for (int k = 0; k < 5; k++) {
-                const u64 m = (u64)(e[k] < 0 ? -e[k] : e[k]);
-                a[k] += m;
-                if (m > 0x7FFFFFFFull) *inv |= 1u << k;
-            }
-        }
-    }
-
     __device__ uint32_t fixed_sums(int c, uint32_t w, uint32_t sb, u64 tot[5], float rb[5])
     {
         u64 a0 = 0, a1 = 0, a2 = 0, a3 = 0, a4 = 0;
         uint32_t order;
         const uint32_t len = n - 4;
         if (sb < 28) {
-            // 32-bit accumulators (exact) while sb + ilog2((n-4)*17) < 32, else the _wide routine: AVX2 lanes, no remainder
-            if ((len & 3) == 0 || sb + ilog2_32(len * 17) < 32) {
-                for (uint32_t i = 4 + lane; i < n; i += 64) {
-                    int32_t v0 = get(c, i, w), v1 = get(c, i - 1, w), v2 = get(c, i - 2, w), v3 = get(c, i - 3, w),
-                            v4 = get(c, i - 4, w);
-                    int32_t e1 = v0 - v1, d1 = v1 - v2, d2 = v2 - v3, d3 = v3 - v4;
-                    int32_t e2 = e1 - d1, f2 = d1 - d2, g2 = d2 - d3;
-                    int32_t e3 = e2 - f2, f3 = f2 - g2;
-                    int32_t e4 = e3 - f3;
-                    a0 += (uint32_t)abs(v0); a1 += (uint32_t)abs(e1); a2 += (uint32_t)abs(e2);
-                    a3 += (uint32_t)abs(e3); a4 += (uint32_t)abs(e4);
-                }
-            }
-            else {
-                u64 a[5] = {0, 0, 0, 0, 0};
-                uint32_t inv = 0;
-                lane_sums(c, w, len, a, &inv);
-                a0 = a[0]; a1 = a[1]; a2 = a[2]; a3 = a[3]; a4 = a[4];
+            // every sample from the fifth on, exact: differences of 27-bit values stay below 2^31
+            for (uint32_t i = 4 + lane; i < n; i += 64) {
+                int32_t v0 = get(c, i, w), v1 = get(c, i - 1, w), v2 = get(c, i - 2, w), v3 = get(c, i - 3, w),
+                        v4 = get(c, i - 4, w);
+                int32_t e1 = v0 - v1, d1 = v1 - v2, d2 = v2 - v3, d3 = v3 - v4;
+                int32_t e2 = e1 - d1, f2 = d1 - d2, g2 = d2 - d3;
+                int32_t e3 = e2 - f2, f3 = f2 - g2;
+                int32_t e4 = e3 - f3;
+                a0 += (uint32_t)abs(v0); a1 += (uint32_t)abs(e1); a2 += (uint32_t)abs(e2);
+                a3 += (uint32_t)abs(e3); a4 += (uint32_t)abs(e4);
             }
             tot[0] = wave_add64(a0); tot[1] = wave_add64(a1); tot[2] = wave_add64(a2);
             tot[3] = wave_add64(a3); tot[4] = wave_add64(a4);
@@ -305,13 +276,10 @@ struct Enc {
                 rb[k] = (float)((tot[k] > 0) ? log(FG_LN2 * (double)tot[k] / dlen) / FG_LN2 : 0.0);
         }
         else {
-            // sbps >= 28: libFLAC's _limit_residual variants (oracle/flac_oracle.c fixed_best_predictor).  33 bit: plain
-            // sums over every sample.  <= 32 bit: warm-up positions + AVX2 lanes + the len%4 samples at the end.
+            // sbps >= 28: libFLAC's _limit_residual rules (oracle/flac_oracle.c fixed_best_predictor): every sample, the
+            // warm-up positions included
             uint32_t inv = 0;
-            const bool lanes = sb <= 32 && (len & 3) != 0;
-            const uint32_t tail0 = 4 + (len & ~3u);
             for (uint32_t i = lane; i < n; i += 64) {
-                if (lanes && i >= 4 && i < tail0) continue;
                 i64 v0 = get64(c, i, w);
                 i64 v1 = i >= 1 ? get64(c, i - 1, w) : 0, v2 = i >= 2 ? get64(c, i - 2, w) : 0;
                 i64 v3 = i >= 3 ? get64(c, i - 3, w) : 0, v4 = i >= 4 ? get64(c, i - 4, w) : 0;
@@ -327,11 +295,6 @@ struct Enc {
                 if (e2 > 0x7FFFFFFFull) inv |= 4;
                 if (e3 > 0x7FFFFFFFull) inv |= 8;
                 if (e4 > 0x7FFFFFFFull) inv |= 16;
-            }
-            if (lanes) {
-                u64 a[5] = {0, 0, 0, 0, 0};
-                lane_sums(c, w, len, a, &inv);
-                a0 += a[0]; a1 += a[1]; a2 += a[2]; a3 += a[3]; a4 += a[4];
             }
             inv = wave_or(inv);
             tot[0] = wave_add64(a0); tot[1] = wave_add64(a1); tot[2] = wave_add64(a2);

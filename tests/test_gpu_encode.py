@@ -730,10 +730,7 @@ def test_ragged_blocks_of_true_32_bit_content_stay_in_the_pipeline(ctx, level):
     """Round 6 (the third time asked): tails and odd block sizes of TRUE 32-bit content -- 33-bit side channel, fewer than eight shared
     wasted bits -- are evaluated and packed by the pipeline's fp64 forms in the ragged lane geometry instead of going to the generic
     kernel.  Stereo and mono, tails of many lengths (one sample more in some lanes of a group, idle lanes, short partitions), an odd
-    block size, a few wasted bits -- and every residue of (length - 4) mod 4: the reference binary sums the fixed predictors' errors
-    with AVX2 routines whose lanes start late against their histories when that residue is 2 or 3 (and which drop, or count twice,
-    the samples at the end); the pipeline reproduces those sums (the first version of these forms did not, and 33 of 2949 fuzz
-    cases on the emulator said so)."""
+    block size, a few wasted bits -- and every residue of (length - 4) mod 4."""
     import torch
     from pyflac_amd import batch
     from oracle import oracle as O
