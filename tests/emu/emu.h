@@ -91,7 +91,7 @@ bool parse_text(CodeObject &co);
     X(s_addk_i32) X(s_mulk_i32) X(s_getpc_b64) X(s_setpc_b64) X(s_swappc_b64) X(s_set_gpr_idx_on) X(s_set_gpr_idx_off) X(s_set_gpr_idx_idx) \
     X(s_branch) X(s_cbranch_scc0) X(s_cbranch_scc1) X(s_cbranch_vccz) X(s_cbranch_vccnz) X(s_cbranch_execz) X(s_cbranch_execnz) \
     X(s_endpgm) X(s_barrier) X(s_waitcnt) X(s_nop) X(s_sleep) X(s_memrealtime) X(s_memtime) X(s_trap) X(s_sethalt) X(s_setprio) X(s_code_end) \
-    X(s_load_dword) X(s_load_dwordx2) X(s_load_dwordx4) X(s_load_dwordx8) X(s_load_dwordx16) X(s_dcache_wb) X(s_dcache_inv) X(s_icache_inv) \
+    X(s_load_dword) X(s_load_dwordx2) X(s_load_dwordx4) X(s_load_dwordx8) X(s_load_dwordx16) X(s_dcache_inv) X(s_icache_inv) \
     X(v_mov_b32) X(v_mov_b64) X(v_add_u32) X(v_sub_u32) X(v_subrev_u32) X(v_add_co_u32) X(v_addc_co_u32) X(v_sub_co_u32) X(v_subb_co_u32) \
     X(v_subrev_co_u32) X(v_subbrev_co_u32) X(v_mul_lo_u32) X(v_mul_hi_u32) X(v_mul_hi_i32) X(v_mul_i32_i24) X(v_mul_u32_u24) X(v_mul_hi_i32_i24) X(v_mul_hi_u32_u24) \
     X(v_mad_i32_i24) X(v_mad_u32_u24) X(v_mad_u64_u32) X(v_mad_i64_i32) X(v_and_b32) X(v_or_b32) X(v_xor_b32) X(v_xnor_b32) X(v_not_b32) \

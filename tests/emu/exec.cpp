@@ -902,7 +902,7 @@ static bool exec_salu(Wave &w, const Inst &in, bool *jumped)
         else if (o[0].kind == K_VCC) w.vcc = (u64)t[0] | ((u64)t[1] << 32);
         else ws32(w, o[0], t[0]);
     } break;
-    case OP_s_waitcnt: case OP_s_nop: case OP_s_setprio: case OP_s_dcache_wb: case OP_s_dcache_inv: case OP_s_icache_inv: case OP_s_sethalt: break;
+    case OP_s_waitcnt: case OP_s_nop: case OP_s_setprio: case OP_s_dcache_inv: case OP_s_icache_inv: case OP_s_sethalt: break;
     case OP_s_trap: emu_fault(w, "s_trap (an assertion or an abort() in device code)"); return false;
     default: emu_fault(w, "scalar instruction not implemented"); return false;
     }

@@ -233,7 +233,7 @@ static bool parse_line(const std::string &line, Inst &in, std::string &err)
     if (op < 0) { err = "unknown mnemonic " + mn; return false; }
     in.op = (u16)op;
     if (in.op == OP_s_waitcnt || in.op == OP_s_nop || in.op == OP_s_endpgm || in.op == OP_s_barrier || in.op == OP_s_code_end ||
-        in.op == OP_buffer_inv || in.op == OP_buffer_wbl2 || in.op == OP_buffer_wbinvl1 || in.op == OP_s_dcache_wb || in.op == OP_s_icache_inv ||
+        in.op == OP_buffer_inv || in.op == OP_buffer_wbl2 || in.op == OP_buffer_wbinvl1 || in.op == OP_s_icache_inv ||
         in.op == OP_s_dcache_inv || in.op == OP_s_set_gpr_idx_off || in.op == OP_s_setprio || in.op == OP_v_nop || in.op == OP_ds_nop) return true;
     if (in.op == OP_s_set_gpr_idx_on) {
         // s_set_gpr_idx_on s62, gpr_idx(DST)   |  gpr_idx(SRC0,DST)
