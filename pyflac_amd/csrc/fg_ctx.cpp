@@ -317,7 +317,7 @@ uint32_t fg_slot_bytes(const flacgpu_settings &s, uint32_t max_n)
     return (uint32_t)((slot + 255) & ~(uint64_t)255);
 }
 
-void fg_fill_params(const flacgpu_settings &s, uint32_t max_n, bool pcm_i16, bool debug, FgEncParams *P)
+void fg_fill_params(const flacgpu_settings &s, uint32_t max_n, bool pcm_i16, FgEncParams *P)
 {
     memset(P, 0, sizeof *P);
     P->channels = s.channels; P->bps = s.bits_per_sample; P->sample_rate = s.sample_rate; P->blocksize = s.blocksize;
@@ -333,8 +333,6 @@ void fg_fill_params(const flacgpu_settings &s, uint32_t max_n, bool pcm_i16, boo
     if (s.apod_parts >= 2) for (uint32_t b = 2; b <= s.apod_parts; b++) nvec += (b == 2) ? 2 : 2 * b;
     P->nvec = nvec;
     P->pcm_i16 = pcm_i16 ? 1 : 0;
-    P->debug = debug ? 1 : 0;
-    if (fg_tune("FLACGPU_STOP")) P->debug = 100 + atoi(fg_tune("FLACGPU_STOP"));
     const uint32_t mo = s.max_lpc_order ? s.max_lpc_order : 1;
     uint32_t dbuf = 4 * (FG_DH + FG_DK) * 8;
     const uint32_t lev = FG_MAX_CAND * nvec * mo * 12 + 64;
@@ -523,7 +521,7 @@ static bool encode_streams_impl(flacgpu_ctx *c, const flacgpu_settings *s, const
     if (s->max_lpc_order == 0 && c->h_windows.empty()) c->window_offset(16, 0);
     if (!c->sync_windows()) return false;
     FgEncParams P;
-    fg_fill_params(*s, s->blocksize, pcm_is_i16 != 0, c->debug, &P);
+    fg_fill_params(*s, s->blocksize, pcm_is_i16 != 0, &P);
     if (fg_enc_lds_bytes(&P) > 64 * 1024) {
         // large blocks: the generic kernel reads the PCM in place instead of staging it in LDS
         if (pcm_is_i16) { fg_set_error("int16 ingest needs blocks that fit LDS"); return false; }

@@ -180,7 +180,7 @@ hipError_t fg_stream_wait(hipStream_t stream);
 
 int fg_resolve_settings(flacgpu_settings *s);
 // settings helpers shared by the libFLAC-style encoder and the batch API
-void fg_fill_params(const flacgpu_settings &s, uint32_t max_n, bool pcm_i16, bool debug, FgEncParams *P);
+void fg_fill_params(const flacgpu_settings &s, uint32_t max_n, bool pcm_i16, FgEncParams *P);
 uint32_t fg_slot_bytes(const flacgpu_settings &s, uint32_t max_n);
 void fg_tukey_window(float *w, int32_t L, float p);
 

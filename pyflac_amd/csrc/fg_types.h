@@ -9,7 +9,7 @@
 //     FLACGPU_DEC_GATE, FLACGPU_DEC_P16, FLACGPU_DEC_WAVE; FLACGPU_WINDOW_SELFTEST, FLACGPU_VERIFY_SELFTEST) are read by the test-hooks library only
 //     (libflacgpu_testhooks.so: the same kernel objects, the three host files compiled with -DFG_TESTHOOKS; the cross-check tests
 //     load it explicitly, pyflac_amd/_lib.py testhooks_lib()).
-//   * fg_tune(): everything that skips work, reorders it for an experiment or prints diagnostics (FLACGPU_DEC_SKIP, FLACGPU_STOP,
+//   * fg_tune(): everything that skips work, reorders it for an experiment or prints diagnostics (FLACGPU_DEC_SKIP,
 //     FLACGPU_DEC_CRC_LATE, FLACGPU_LDS_PAD, FLACGPU_FCAP, FLACGPU_ALIAS, FLACGPU_DIRECT_X, FLACGPU_SPIN_US,
 //     FLACGPU_DEC_PROF, FLACGPU_API_PROF, FG_REFWALK_DEBUG, FLACGPU_DEC_WPS) is read by `make TUNING=1` builds only.
 // flacgpu_build_flags() says what a library is: bit 0 tuning, bit 2 test hooks.
@@ -62,7 +62,6 @@ struct FgEncParams {
     uint32_t sig_stride;   // int32 elements per staged channel in LDS
     uint32_t nvec;         // autocorrelation vectors per candidate
     uint32_t pcm_i16;      // input is interleaved int16 instead of int32
-    uint32_t debug;
     uint32_t lds_dbuf_bytes;
     uint32_t limit_min_bitrate;   // a frame may not consist of CONSTANT subframes only (see the kernels' baseline stage)
 };

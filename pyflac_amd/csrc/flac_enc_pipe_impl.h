@@ -41,12 +41,6 @@
 #define LDS __attribute__((address_space(3)))
 #define FGI __device__ __forceinline__
 
-// (P.debug values 101..103 switch parts of the autocorrelation kernel off: timing experiments of round 3, compiled into tuning builds only)
-#ifdef FG_TUNING
-#define FGX_DBG(v) (P.debug == (v))
-#else
-#define FGX_DBG(v) false
-#endif
 #ifndef FGX_AUTOC_RD2
 #define FGX_AUTOC_RD2 1
 #endif
@@ -374,15 +368,14 @@ fg_pipe_autoc_kernel(const void *pcm, const FgBlockDesc *descs, const float *win
 #pragma unroll
                         for (int u = 0; u < FGP_CK / 64; u++) {
                             const uint32_t j = u * 64 + lane;
-                            if (!FGX_DBG(102)) {       // (behind the end of the signal the fetch gave zeros: the chains run on a little)
-                                int32_t L = xl[u], R = xr[u];
-                                unraw(L, R);
+                            // (behind the end of the signal the fetch gave zeros: the chains run on a little)
+                            int32_t L = xl[u], R = xr[u];
+                            unraw(L, R);
 #pragma unroll
-                                for (int c = 0; c < NC; c++) {
-                                    const int32_t x = c == 0 ? pcv<MS, 0>(L, R) : c == 1 ? pcv<MS, 1>(L, R) : c == 2 ? pcv<MS, 2>(L, R) : pcv<MS, 3>(L, R);
-                                    orv[c] |= (uint32_t)x;       // (windows after the first see samples the first has seen: the OR stands)
-                                    dbuf[c * FGP_CSTR + FGP_DH + j] = (double)((float)x * wv[u]);
-                                }
+                            for (int c = 0; c < NC; c++) {
+                                const int32_t x = c == 0 ? pcv<MS, 0>(L, R) : c == 1 ? pcv<MS, 1>(L, R) : c == 2 ? pcv<MS, 2>(L, R) : pcv<MS, 3>(L, R);
+                                orv[c] |= (uint32_t)x;       // (windows after the first see samples the first has seen: the OR stands)
+                                dbuf[c * FGP_CSTR + FGP_DH + j] = (double)((float)x * wv[u]);
                             }
                         }
                     }
@@ -390,47 +383,44 @@ fg_pipe_autoc_kernel(const void *pcm, const FgBlockDesc *descs, const float *win
 #pragma unroll
                         for (int u = 0; u < FGP_CK / 64; u++) {
                             const uint32_t j = u * 64 + lane;
-                            if (!FGX_DBG(102)) {
-                                int32_t L = xl[u], R = xr[u];
-                                unraw(L, R);
-                                const bool zero = part != 0 && (k0 + j) >= 2 * part;
+                            int32_t L = xl[u], R = xr[u];
+                            unraw(L, R);
+                            const bool zero = part != 0 && (k0 + j) >= 2 * part;
 #pragma unroll
-                                for (int c = 0; c < NC; c++) {
-                                    float fx;
-                                    uint32_t ob;
-                                    cval(c, L, R, fx, ob);
-                                    if (nv == 0) orv[c] |= ob;
-                                    const float dd = zero ? 0.0f : fx * wv[u];
-                                    dbuf[c * FGP_CSTR + FGP_DH + j] = (double)dd;
-                                }
+                            for (int c = 0; c < NC; c++) {
+                                float fx;
+                                uint32_t ob;
+                                cval(c, L, R, fx, ob);
+                                if (nv == 0) orv[c] |= ob;
+                                const float dd = zero ? 0.0f : fx * wv[u];
+                                dbuf[c * FGP_CSTR + FGP_DH + j] = (double)dd;
                             }
                         }
                     }
                     if (k0 + FGP_CK < vec_len) fetch(k0 + FGP_CK);
                     wave_lds_fence();
-                    if (!FGX_DBG(101)) {
-                        // The chains on the matrix core.  v_mfma_f64_4x4x4_4b_f64 computes, for four independent blocks b,
-                        // D[i][j] += sum_k A[i][k] * B[k][j] with one fused multiply-add per k, in ascending k, each rounded like
-                        // v_fma_f64 (tools/ubench/mfma64.hip: 262144 random cases bit-equal to that chain and to no other
-                        // order).  Lanes: A and B in lane k*16 + b*4 + x (x = i resp. j), D in lane i*16 + b*4 + j.  With
-                        //     A[i][k] = d[t + k - i]        B[k][j] = d[t + k - 4j]
-                        // one instruction adds steps t .. t+3, in order, to the chains of lags 4j - i = -3 .. 12 of the four
-                        // candidates b: 256 of libFLAC's fused multiply-adds, in libFLAC's order per lag (row i runs i steps
-                        // behind; zeros in front of the signal and behind it add nothing; lags -1 .. -3 repeat 1 .. 3 and are
-                        // dropped).  A comes from LDS (one ds_read_b64 per instruction).  B of the next step group is B of this
-                        // one moved up a lane inside each quad, with the A just read entering at j = 0 (the same d[t + k]):
-                        // two v_cndmask_b32_dpp.
-                        const uint32_t kend = (k0 + kn < vec_len) ? FGP_CK : ((kn + 3) & ~3u) + 4;
-                        const LDS double *pa = dbuf + mrow * FGP_CSTR + FGP_DH + (lane >> 4) - (lane & 3);
-                        // One asm block per chunk (fixed registers v40..v59: A of two groups of four instructions in flight,
-                        // B alternating between two pairs so that no instruction overwrites an operand of the one before it).
-                        // Wait states by hand -- the compiler's hazard recogniser does not look inside: a dependent
-                        // v_mfma_f64_4x4x4 needs 4 after the one that wrote its accumulator (two v_cndmask + s_nop 1), its
-                        // result 9+ before anything else reads it (the s_nop at the end).
-                        uint32_t ad = (uint32_t)(size_t)pa;
-                        const uint32_t adb = ad - 8u * (4u + 3u * (lane & 3));        // d[-4 + k - 4j]: B of the step group before the chunk
-                        uint32_t n4 = kend >> 4, n1 = (kend >> 2) & 3;
-                        const u64 m0 = 0x1111111111111111ull;                          // lanes with j = 0
+                    // The chains on the matrix core.  v_mfma_f64_4x4x4_4b_f64 computes, for four independent blocks b,
+                    // D[i][j] += sum_k A[i][k] * B[k][j] with one fused multiply-add per k, in ascending k, each rounded like
+                    // v_fma_f64 (tools/ubench/mfma64.hip: 262144 random cases bit-equal to that chain and to no other
+                    // order).  Lanes: A and B in lane k*16 + b*4 + x (x = i resp. j), D in lane i*16 + b*4 + j.  With
+                    //     A[i][k] = d[t + k - i]        B[k][j] = d[t + k - 4j]
+                    // one instruction adds steps t .. t+3, in order, to the chains of lags 4j - i = -3 .. 12 of the four
+                    // candidates b: 256 of libFLAC's fused multiply-adds, in libFLAC's order per lag (row i runs i steps
+                    // behind; zeros in front of the signal and behind it add nothing; lags -1 .. -3 repeat 1 .. 3 and are
+                    // dropped).  A comes from LDS (one ds_read_b64 per instruction).  B of the next step group is B of this
+                    // one moved up a lane inside each quad, with the A just read entering at j = 0 (the same d[t + k]):
+                    // two v_cndmask_b32_dpp.
+                    const uint32_t kend = (k0 + kn < vec_len) ? FGP_CK : ((kn + 3) & ~3u) + 4;
+                    const LDS double *pa = dbuf + mrow * FGP_CSTR + FGP_DH + (lane >> 4) - (lane & 3);
+                    // One asm block per chunk (fixed registers v40..v59: A of two groups of four instructions in flight,
+                    // B alternating between two pairs so that no instruction overwrites an operand of the one before it).
+                    // Wait states by hand -- the compiler's hazard recogniser does not look inside: a dependent
+                    // v_mfma_f64_4x4x4 needs 4 after the one that wrote its accumulator (two v_cndmask + s_nop 1), its
+                    // result 9+ before anything else reads it (the s_nop at the end).
+                    uint32_t ad = (uint32_t)(size_t)pa;
+                    const uint32_t adb = ad - 8u * (4u + 3u * (lane & 3));        // d[-4 + k - 4j]: B of the step group before the chunk
+                    uint32_t n4 = kend >> 4, n1 = (kend >> 2) & 3;
+                    const u64 m0 = 0x1111111111111111ull;                          // lanes with j = 0
 #define FG_DPPQ " quad_perm:[0,0,1,2] row_mask:0xf bank_mask:0xf\n\t"
 #define FG_STEP(a0, a1, s0, s1, d0, d1) \
     "v_cndmask_b32_dpp v" #d0 ", v" #s0 ", v" #a0 ", vcc" FG_DPPQ \
@@ -445,95 +435,95 @@ fg_pipe_autoc_kernel(const void *pcm, const FgBlockDesc *descs, const float *win
 #define FG_EVEN(a0, a1) FG_STEP(a0, a1, 56, 57, 58, 59)
 #define FG_ODD(a0, a1) FG_STEP(a0, a1, 58, 59, 56, 57)
 #if FGX_AUTOC_RD2
-                        // (round 5: A of two groups of TWO instructions in flight -- v40..v47 -- instead of two groups of four: eight
-                        // registers fewer are out of the compiler's reach, and the kernel no longer spills -- 100 bytes of scratch a lane
-                        // were 45 MB written and about as much read back per launch)
-                        asm volatile(
-                            "s_mov_b64 vcc, %[m0]\n\t"
-                            "ds_read_b64 v[56:57], %[adb]\n\t"
-                            "s_cmp_eq_u32 %[n4], 0\n\t"
-                            "s_cbranch_scc1 2f\n\t"
-                            FG_RD2(40, 41, 42, 43, 0)
-                            "1:\n\t"
-                            FG_RD2(44, 45, 46, 47, 64)
-                            "s_waitcnt lgkmcnt(2)\n\t"
-                            FG_EVEN(40, 41) FG_ODD(42, 43)
-                            "v_add_u32 %[ad], 0x80, %[ad]\n\t"
-                            "s_sub_u32 %[n4], %[n4], 1\n\t"
-                            "s_cmp_eq_u32 %[n4], 0\n\t"
-                            "s_cbranch_scc1 5f\n\t"
-                            FG_RD2(40, 41, 42, 43, 0)
-                            "s_waitcnt lgkmcnt(2)\n\t"
-                            FG_EVEN(44, 45) FG_ODD(46, 47)
-                            "s_branch 1b\n\t"
-                            "5:\n\t"
-                            "s_waitcnt lgkmcnt(0)\n\t"
-                            FG_EVEN(44, 45) FG_ODD(46, 47)
-                            "2:\n\t"
-                            "s_waitcnt lgkmcnt(0)\n\t"
-                            "s_cmp_eq_u32 %[n1], 0\n\t"
-                            "s_cbranch_scc1 4f\n\t"
-                            "3:\n\t"
-                            "ds_read_b64 v[40:41], %[ad]\n\t"
-                            "v_add_u32 %[ad], 32, %[ad]\n\t"
-                            "s_sub_u32 %[n1], %[n1], 1\n\t"
-                            "s_waitcnt lgkmcnt(0)\n\t"
-                            FG_EVEN(40, 41)
-                            "v_mov_b32 v56, v58\n\t"
-                            "v_mov_b32 v57, v59\n\t"
-                            "s_nop 1\n\t"
-                            "s_cmp_eq_u32 %[n1], 0\n\t"
-                            "s_cbranch_scc0 3b\n\t"
-                            "4:\n\t"
-                            "s_nop 7\n\t"
-                            "s_nop 3"
-                            : [acc] "+v"(acc), [ad] "+v"(ad), [n4] "+s"(n4), [n1] "+s"(n1)
-                            : [adb] "v"(adb), [m0] "s"(m0)
-                            : "vcc", "scc", "memory", "v40", "v41", "v42", "v43", "v44", "v45", "v46", "v47", "v56", "v57", "v58", "v59");
+                    // (round 5: A of two groups of TWO instructions in flight -- v40..v47 -- instead of two groups of four: eight
+                    // registers fewer are out of the compiler's reach, and the kernel no longer spills -- 100 bytes of scratch a lane
+                    // were 45 MB written and about as much read back per launch)
+                    asm volatile(
+                        "s_mov_b64 vcc, %[m0]\n\t"
+                        "ds_read_b64 v[56:57], %[adb]\n\t"
+                        "s_cmp_eq_u32 %[n4], 0\n\t"
+                        "s_cbranch_scc1 2f\n\t"
+                        FG_RD2(40, 41, 42, 43, 0)
+                        "1:\n\t"
+                        FG_RD2(44, 45, 46, 47, 64)
+                        "s_waitcnt lgkmcnt(2)\n\t"
+                        FG_EVEN(40, 41) FG_ODD(42, 43)
+                        "v_add_u32 %[ad], 0x80, %[ad]\n\t"
+                        "s_sub_u32 %[n4], %[n4], 1\n\t"
+                        "s_cmp_eq_u32 %[n4], 0\n\t"
+                        "s_cbranch_scc1 5f\n\t"
+                        FG_RD2(40, 41, 42, 43, 0)
+                        "s_waitcnt lgkmcnt(2)\n\t"
+                        FG_EVEN(44, 45) FG_ODD(46, 47)
+                        "s_branch 1b\n\t"
+                        "5:\n\t"
+                        "s_waitcnt lgkmcnt(0)\n\t"
+                        FG_EVEN(44, 45) FG_ODD(46, 47)
+                        "2:\n\t"
+                        "s_waitcnt lgkmcnt(0)\n\t"
+                        "s_cmp_eq_u32 %[n1], 0\n\t"
+                        "s_cbranch_scc1 4f\n\t"
+                        "3:\n\t"
+                        "ds_read_b64 v[40:41], %[ad]\n\t"
+                        "v_add_u32 %[ad], 32, %[ad]\n\t"
+                        "s_sub_u32 %[n1], %[n1], 1\n\t"
+                        "s_waitcnt lgkmcnt(0)\n\t"
+                        FG_EVEN(40, 41)
+                        "v_mov_b32 v56, v58\n\t"
+                        "v_mov_b32 v57, v59\n\t"
+                        "s_nop 1\n\t"
+                        "s_cmp_eq_u32 %[n1], 0\n\t"
+                        "s_cbranch_scc0 3b\n\t"
+                        "4:\n\t"
+                        "s_nop 7\n\t"
+                        "s_nop 3"
+                        : [acc] "+v"(acc), [ad] "+v"(ad), [n4] "+s"(n4), [n1] "+s"(n1)
+                        : [adb] "v"(adb), [m0] "s"(m0)
+                        : "vcc", "scc", "memory", "v40", "v41", "v42", "v43", "v44", "v45", "v46", "v47", "v56", "v57", "v58", "v59");
 #else
-                        asm volatile(
-                            "s_mov_b64 vcc, %[m0]\n\t"
-                            "ds_read_b64 v[56:57], %[adb]\n\t"
-                            "s_cmp_eq_u32 %[n4], 0\n\t"
-                            "s_cbranch_scc1 2f\n\t"
-                            FG_RD4(40, 41, 42, 43, 44, 45, 46, 47, 0)
-                            "1:\n\t"
-                            FG_RD4(48, 49, 50, 51, 52, 53, 54, 55, 128)
-                            "s_waitcnt lgkmcnt(4)\n\t"
-                            FG_EVEN(40, 41) FG_ODD(42, 43) FG_EVEN(44, 45) FG_ODD(46, 47)
-                            "v_add_u32 %[ad], 0x80, %[ad]\n\t"
-                            "s_sub_u32 %[n4], %[n4], 1\n\t"
-                            "s_cmp_eq_u32 %[n4], 0\n\t"
-                            "s_cbranch_scc1 2f\n\t"
-                            FG_RD4(40, 41, 42, 43, 44, 45, 46, 47, 128)
-                            "s_waitcnt lgkmcnt(4)\n\t"
-                            FG_EVEN(48, 49) FG_ODD(50, 51) FG_EVEN(52, 53) FG_ODD(54, 55)
-                            "v_add_u32 %[ad], 0x80, %[ad]\n\t"
-                            "s_sub_u32 %[n4], %[n4], 1\n\t"
-                            "s_cmp_eq_u32 %[n4], 0\n\t"
-                            "s_cbranch_scc0 1b\n\t"
-                            "2:\n\t"
-                            "s_waitcnt lgkmcnt(0)\n\t"
-                            "s_cmp_eq_u32 %[n1], 0\n\t"
-                            "s_cbranch_scc1 4f\n\t"
-                            "3:\n\t"
-                            "ds_read_b64 v[40:41], %[ad]\n\t"
-                            "v_add_u32 %[ad], 32, %[ad]\n\t"
-                            "s_sub_u32 %[n1], %[n1], 1\n\t"
-                            "s_waitcnt lgkmcnt(0)\n\t"
-                            FG_EVEN(40, 41)
-                            "v_mov_b32 v56, v58\n\t"
-                            "v_mov_b32 v57, v59\n\t"
-                            "s_nop 1\n\t"
-                            "s_cmp_eq_u32 %[n1], 0\n\t"
-                            "s_cbranch_scc0 3b\n\t"
-                            "4:\n\t"
-                            "s_nop 7\n\t"
-                            "s_nop 3"
-                            : [acc] "+v"(acc), [ad] "+v"(ad), [n4] "+s"(n4), [n1] "+s"(n1)
-                            : [adb] "v"(adb), [m0] "s"(m0)
-                            : "vcc", "scc", "memory", "v40", "v41", "v42", "v43", "v44", "v45", "v46", "v47", "v48", "v49", "v50", "v51", "v52", "v53",
-                              "v54", "v55", "v56", "v57", "v58", "v59");
+                    asm volatile(
+                        "s_mov_b64 vcc, %[m0]\n\t"
+                        "ds_read_b64 v[56:57], %[adb]\n\t"
+                        "s_cmp_eq_u32 %[n4], 0\n\t"
+                        "s_cbranch_scc1 2f\n\t"
+                        FG_RD4(40, 41, 42, 43, 44, 45, 46, 47, 0)
+                        "1:\n\t"
+                        FG_RD4(48, 49, 50, 51, 52, 53, 54, 55, 128)
+                        "s_waitcnt lgkmcnt(4)\n\t"
+                        FG_EVEN(40, 41) FG_ODD(42, 43) FG_EVEN(44, 45) FG_ODD(46, 47)
+                        "v_add_u32 %[ad], 0x80, %[ad]\n\t"
+                        "s_sub_u32 %[n4], %[n4], 1\n\t"
+                        "s_cmp_eq_u32 %[n4], 0\n\t"
+                        "s_cbranch_scc1 2f\n\t"
+                        FG_RD4(40, 41, 42, 43, 44, 45, 46, 47, 128)
+                        "s_waitcnt lgkmcnt(4)\n\t"
+                        FG_EVEN(48, 49) FG_ODD(50, 51) FG_EVEN(52, 53) FG_ODD(54, 55)
+                        "v_add_u32 %[ad], 0x80, %[ad]\n\t"
+                        "s_sub_u32 %[n4], %[n4], 1\n\t"
+                        "s_cmp_eq_u32 %[n4], 0\n\t"
+                        "s_cbranch_scc0 1b\n\t"
+                        "2:\n\t"
+                        "s_waitcnt lgkmcnt(0)\n\t"
+                        "s_cmp_eq_u32 %[n1], 0\n\t"
+                        "s_cbranch_scc1 4f\n\t"
+                        "3:\n\t"
+                        "ds_read_b64 v[40:41], %[ad]\n\t"
+                        "v_add_u32 %[ad], 32, %[ad]\n\t"
+                        "s_sub_u32 %[n1], %[n1], 1\n\t"
+                        "s_waitcnt lgkmcnt(0)\n\t"
+                        FG_EVEN(40, 41)
+                        "v_mov_b32 v56, v58\n\t"
+                        "v_mov_b32 v57, v59\n\t"
+                        "s_nop 1\n\t"
+                        "s_cmp_eq_u32 %[n1], 0\n\t"
+                        "s_cbranch_scc0 3b\n\t"
+                        "4:\n\t"
+                        "s_nop 7\n\t"
+                        "s_nop 3"
+                        : [acc] "+v"(acc), [ad] "+v"(ad), [n4] "+s"(n4), [n1] "+s"(n1)
+                        : [adb] "v"(adb), [m0] "s"(m0)
+                        : "vcc", "scc", "memory", "v40", "v41", "v42", "v43", "v44", "v45", "v46", "v47", "v48", "v49", "v50", "v51", "v52", "v53",
+                          "v54", "v55", "v56", "v57", "v58", "v59");
 #endif
 #undef FG_RD2
 #undef FG_EVEN
@@ -541,9 +531,8 @@ fg_pipe_autoc_kernel(const void *pcm, const FgBlockDesc *descs, const float *win
 #undef FG_RD4
 #undef FG_STEP
 #undef FG_DPPQ
-                    }
                     wave_lds_fence();
-                    if (k0 + kn < vec_len && !FGX_DBG(103)) {
+                    if (k0 + kn < vec_len) {
                         double t[(NC * FGP_DH + 63) / 64];
 #pragma unroll
                         for (int u = 0; u < (NC * FGP_DH + 63) / 64; u++) {

@@ -497,7 +497,7 @@ FLAC__StreamEncoderInitStatus init_common(EncImpl *e)
     e->ctx = fg_default_ctx();
     if (!e->ctx) return FLAC__STREAM_ENCODER_INIT_STATUS_ENCODER_ERROR;
     FgEncParams P;
-    fg_fill_params(s, s.blocksize, false, false, &P);
+    fg_fill_params(s, s.blocksize, false, &P);
     P.sig_stride = 0;   // worst case: samples read in place
     if (fg_enc_lds_bytes(&P) > 160 * 1024) {
         fg_set_error("settings need more LDS than the device has");

@@ -35,3 +35,8 @@ def test_the_walk_finds_the_sources():
 def test_nothing_writes_through_the_scalar_data_cache(pattern):
     """No kernel here does, and the emulator's opcode table does not know such an instruction: it would report one as unknown."""
     assert _holders(pattern) == []
+
+
+@pytest.mark.parametrize('pattern', ['FLACGPU_' + 'STOP', 'FGX_' + 'DBG'])
+def test_no_switch_ends_a_launch_after_a_stage(pattern):
+    assert _holders(pattern) == []
