@@ -158,8 +158,8 @@ def cpu_baseline(pcm16, level, sr, budget_s=12.0, all_cores=True, what='the same
                           'how': 'one oracle process per host core, about 3 s of encodes each, aggregate over the slowest worker'}
                          if all_cores else 'not run in the N > 1 line (the other ranks start up on the same cores); see the N = 1 line',
             'sample': '%.0f s of %s x%d encode / x%d decode passes, MD5 off, 1 thread; '
-                      'oracle/flac_oracle.c is a scalar restatement of libFLAC 1.4.3 (the reference binary does not '
-                      'travel to the GPU box; reference_binary_ratio has what it measured against the oracle)' %
+                      'oracle/flac_oracle.c is a scalar restatement of libFLAC 1.4.3 (the reference binary is not '
+                      'run; reference_binary_ratio has what it once measured against the oracle)' %
                       (a32.shape[0] / sr, what, reps, dreps),
             'wall_s': round(time.perf_counter() - t0, 1)}
 
@@ -814,7 +814,7 @@ def main():
                 res['cpu_baseline']['reference_binary_ratio'] = {
                     'encode': ratio['reference_over_oracle_encode'], 'decode': ratio['reference_over_oracle_decode'],
                     'reference_encode_msamples_per_s_build_container': ratio['reference_encode_msamples_per_s'],
-                    'measured_by': ratio['command'] + ' (build container; the binary does not travel): profiles/r02_cpu_ref_ratio.json'}
+                    'measured_by': 'recorded once, the binary is not run any more: profiles/r02_cpu_ref_ratio.json'}
         print(json.dumps(res))
     if world > 1:
         dist.destroy_process_group()

@@ -10,11 +10,8 @@
  * pyflac/include/FLAC/format.h:191-484,536-557; level presets from
  * pyflac/include/FLAC/stream_encoder.h:845-853).
  *
- * Pinning: tests/test_oracle_vs_reference.py drives the reference's bundled
- * binary (pyflac/libraries/linux-x86_64/libFLAC-12.1.0.so) through
- * oracle/libflac_ref.py in the build container and requires byte-identical
- * output; tests/golden/ holds vectors generated from that binary
- * (oracle/gen_golden.py) so the pin travels to the GPU box.
+ * Pinning: tests/golden/ holds vectors recorded from the library that the
+ * reference bundles; that library itself is neither loaded nor run.
  *
  * Only tests/, __graft_entry__.smoke() and bench.py's cpu_baseline leg may
  * use this code.  The product (pyflac_amd/) never links or calls it.

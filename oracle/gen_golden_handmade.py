@@ -1,23 +1,15 @@
-"""Generate tests/golden/handmade_streams.npz: FLAC streams that libFLAC's encoder never writes but its decoder accepts.
+"""A writer of FLAC streams that libFLAC's encoder never writes but its decoder accepts.
 
-Run in the build container only (needs /root/reference):  python -m oracle.gen_golden_handmade
 A small bit writer assembles frames with features outside the encoder presets: escape-coded (raw) Rice partitions with
 0..24 raw bits under both coding methods, partition order 8, LPC order 32 with 15-bit coefficients and shift 0, variable
 block sizes with every block-size / sample-rate header form and multi-byte sample numbers, wasted bits, verbatim and
-constant subframes in all stereo assignments, 8 channels.  Each stream is decoded with the reference's libFLAC 1.4.3 binary
-(pyflac/decoder.py:170-196 path); the stream and the PCM it returned are stored, so the decoders under test (oracle, GPU)
-are checked against the reference on inputs their own encoders cannot produce.
+constant subframes in all stereo assignments, 8 channels.  tests/golden/handmade_streams.npz holds the streams of
+build_streams() and the PCM recorded for them, which equals the construction: the decoders under test (oracle, GPU) are
+checked on inputs their own encoders cannot produce.
 """
-import os
-import sys
-
 import numpy as np
 
-sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
-
-from oracle import libflac_ref as R  # noqa: E402
-from oracle import oracle as O  # noqa: E402
-from tests import cases  # noqa: E402
+from oracle import oracle as O
 
 
 class BW:
@@ -297,19 +289,3 @@ def build_streams():
     out['side33'] = (streaminfo(1024, 1024, 48000, 2, 32, 1024 * 4) + b''.join(frames), np.concatenate(pcms))
     return out
 
-
-def main():
-    streams = build_streams()
-    store = {}
-    for name, (data, pcm) in sorted(streams.items()):
-        got, frames, st = R.decode(data, want_frames=False)
-        ok = not st['errors'] and got.shape == pcm.shape and np.array_equal(got, pcm.astype(np.int32).reshape(got.shape))
-        print('%-12s %7d bytes %3d frames  reference decode %s' % (name, len(data), len(frames), 'matches the construction' if ok else 'DIFFERS: %s' % st))
-        assert ok, name
-        store[name + '.flac'] = np.frombuffer(data, np.uint8)
-        store[name + '.pcm'] = got.astype(np.int32)
-    np.savez_compressed(os.path.join(cases.GOLDEN, 'handmade_streams.npz'), **store)
-
-
-if __name__ == '__main__':
-    main()

@@ -1,4 +1,4 @@
-"""Seeded parity cases shared by the golden generator (oracle/gen_golden.py) and the tests.
+"""Seeded parity cases of the golden vectors and the tests.
 
 Every case is a deterministic PCM generator + encoder settings.  Expected outputs of the
 reference's libFLAC 1.4.3 binary for these cases are committed in tests/golden/encode_vectors.json.
@@ -133,7 +133,7 @@ for _lv in range(9):
 
 
 # FLAC__stream_encoder_set_limit_min_bitrate(true): name -> (pcm spec, sample rate, level, blocksize).
-# Goldens in tests/golden/limit_vectors.json (reference binary, oracle/gen_golden.py).
+# Goldens in tests/golden/limit_vectors.json (recorded from the reference binary).
 _N = 4096 * 5 + 300
 LIMIT_CASES = {
     'lmb_zeros_mono_l5': ({'kind': 'constmix', 'n': _N, 'chans': ['z']}, 48000, 5, 4096),
@@ -228,7 +228,7 @@ def fuzz_damaged_stream(seed):
 
 # Small streams: frames of 10..60 bytes read in answers of a few bytes to a few hundred, so that the refills of libFLAC's reader
 # fall everywhere around the damaged frames (round 3's replay walked in a circle when a refill fell 2..7 bytes behind a damaged
-# frame's sync code; tests/tools/refwalk_small_fuzz.py found 44 such seeds and 8 wrong sequences in its first 3000).  The
+# frame's sync code; 44 such seeds and 8 wrong sequences in the first 3000).  The
 # streams come from the oracle's encoder; the vectors pin them by hash.
 SMALL_DAMAGE_SEEDS = sorted(set(list(range(0, 152)) + [
     82, 95, 417, 433, 499, 501, 531, 570, 651, 721, 885, 909, 929, 966, 1012, 1066, 1114, 1142, 1152, 1174, 1255, 1274, 1275, 1285,

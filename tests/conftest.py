@@ -42,7 +42,7 @@ def damage_golden():
 @pytest.fixture(scope='session')
 def handmade_streams():
     """Streams outside any encoder's repertoire with the PCM the reference binary decoded from them
-    (oracle/gen_golden_handmade.py): name -> (stream bytes, pcm int32[n, ch])."""
+    (the writer: oracle/gen_golden_handmade.py): name -> (stream bytes, pcm int32[n, ch])."""
     import numpy as np
     from tests import cases
     z = np.load(os.path.join(cases.GOLDEN, 'handmade_streams.npz'))
@@ -51,7 +51,7 @@ def handmade_streams():
 
 @pytest.fixture(scope='session')
 def fuzz_golden():
-    """Reference hashes of the seeded random corpus (tests/fuzzgen.py seeds 0..GOLDEN_SEEDS-1; oracle/gen_golden.py)."""
+    """Reference hashes of the seeded random corpus (tests/fuzzgen.py seeds 0..GOLDEN_SEEDS-1)."""
     import json
     from tests import cases
     with open(os.path.join(cases.GOLDEN, 'fuzz_vectors.json')) as f:

@@ -2,8 +2,7 @@
 pyflac/builder/decoder.py:146-231) and a reader of one FLAC__Subframe into plain Python values.
 
 Test infrastructure: what a libFLAC client reads in its write callback.  Used by the GPU tests of FLAC__Frame.subframes[]
-(tests/test_gpu_api.py::TestSubframes) against libflacgpu.so, and by oracle/libflac_ref.py against the reference's binary in
-the build container -- the same structs on both sides."""
+(tests/test_gpu_api.py::TestSubframes) against libflacgpu.so."""
 import ctypes as C
 
 import numpy as np

@@ -1,5 +1,5 @@
 """Builders of FLAC__StreamMetadata blocks (ctypes mirrors in tests/abi_decode.py) for FLAC__stream_encoder_set_metadata:
-the same objects are handed to the reference binary (oracle/gen_golden_setmeta.py, build container) and to libflacgpu
+the same objects were handed to the reference binary (tests/golden/setmeta_vectors.json) and are handed to libflacgpu
 (tests/test_gpu_api.py); what each writes during init_stream is compared byte for byte."""
 import ctypes as C
 

@@ -40,3 +40,7 @@ def test_nothing_writes_through_the_scalar_data_cache(pattern):
 @pytest.mark.parametrize('pattern', ['FLACGPU_' + 'STOP', 'FGX_' + 'DBG'])
 def test_no_switch_ends_a_launch_after_a_stage(pattern):
     assert _holders(pattern) == []
+
+
+def test_no_source_names_a_prebuilt_library_of_the_reference():
+    assert _holders(r'lib' + r'FLAC[-\d.]*\.(so|dll|dylib)') == []

@@ -1,5 +1,4 @@
-"""Edge cases at the limits of the format: GPU encoder vs CPU oracle (and, where /root/reference exists, the oracle vs
-the reference binary).  usage: python tests/tools/extremes.py [ref|gpu]"""
+"""Edge cases at the limits of the format: GPU encoder vs CPU oracle.  usage: python tests/tools/extremes.py"""
 import os, sys
 import numpy as np
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.dirname(os.path.abspath(__file__)))))
@@ -41,48 +40,31 @@ CASES = [
 
 
 def main():
-    mode = sys.argv[1] if len(sys.argv) > 1 else 'gpu'
+    import torch
+    from pyflac_amd import batch
+    from pyflac_amd.encoder import stream_header_bytes
     bad = 0
-    if mode == 'gpu':
-        import torch
-        from pyflac_amd import batch
-        from pyflac_amd.encoder import stream_header_bytes
-        ctx = batch.Context(0)
-    else:
-        from oracle import libflac_ref as R
+    ctx = batch.Context(0)
     for name, n, ch, bps, sr, level, bs, subset, kind in CASES:
         pcm = sig(n, ch, bps, kind)
         cfg, rc = O.config(level, ch, bps, sr, bs, subset)
         a32 = np.ascontiguousarray(pcm.astype(np.int32))
-        if mode == 'ref':
-            arr = pcm.astype(np.int16 if bps == 16 else np.int32)
-            cbs, info = R.encode(arr, sr, bps=bps, level=level, blocksize=bs, extra=None if subset else [('set_streamable_subset', 0)])
-            if rc != info['init_status']:
-                print('INIT', name, rc, info['init_status']); bad += 1
-                continue
-            if rc:
-                print('%-28s init status %d (both)' % (name, rc)); continue
-            want = b''.join(c[0] for c in cbs)
-            got, _ = O.encode_stream(cfg, a32)
-            out, res = O.decode_stream(want)
-            ok = got == want and res.n_errors == 0 and np.array_equal(out.reshape(a32.shape), a32)
-        else:
-            try:
-                s = batch.settings(level, ch, bps, sr, bs, subset)
-                grc = 0
-            except batch.FlacGpuError:
-                grc = 1
-            if (rc != 0) != (grc != 0):
-                print('INIT', name, rc, grc); bad += 1
-                continue
-            if rc:
-                print('%-28s init status %d (both)' % (name, rc)); continue
-            want, _ = O.encode_stream(cfg, a32)
-            t = torch.from_numpy(a32).cuda()
-            out, offs, st = ctx.encode(s, t)
-            got = stream_header_bytes(s) + out[:st.total_bytes].cpu().numpy().tobytes()
-            dec, status, _ = ctx.decode(out[:st.total_bytes], offs, ch, bps, n)
-            ok = got == want and int(status[:, 0].max()) == 0 and torch.equal(dec.reshape(-1, ch), t)
+        try:
+            s = batch.settings(level, ch, bps, sr, bs, subset)
+            grc = 0
+        except batch.FlacGpuError:
+            grc = 1
+        if (rc != 0) != (grc != 0):
+            print('INIT', name, rc, grc); bad += 1
+            continue
+        if rc:
+            print('%-28s init status %d (both)' % (name, rc)); continue
+        want, _ = O.encode_stream(cfg, a32)
+        t = torch.from_numpy(a32).cuda()
+        out, offs, st = ctx.encode(s, t)
+        got = stream_header_bytes(s) + out[:st.total_bytes].cpu().numpy().tobytes()
+        dec, status, _ = ctx.decode(out[:st.total_bytes], offs, ch, bps, n)
+        ok = got == want and int(status[:, 0].max()) == 0 and torch.equal(dec.reshape(-1, ch), t)
         print('%-28s %s (%d bytes)' % (name, 'ok' if ok else 'DIFF', len(want)))
         bad += 0 if ok else 1
     print('%d bad' % bad)
