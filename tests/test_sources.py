@@ -1,10 +1,13 @@
 """What the sources of this repository do not hold."""
 import os
 import re
+import shutil
+import subprocess
 
 import pytest
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+OBJDUMP = '/opt/rocm/lib/llvm/bin/llvm-objdump'
 KINDS = ('.h', '.c', '.cpp', '.hip', '.inc', '.s', '.py', '.sh')
 
 
@@ -44,3 +47,22 @@ def test_no_switch_ends_a_launch_after_a_stage(pattern):
 
 def test_no_source_names_a_prebuilt_library_of_the_reference():
     assert _holders(r'lib' + r'FLAC[-\d.]*\.(so|dll|dylib)') == []
+
+
+def test_packed_fp32_is_neither_written_nor_compiled():
+    """Some packed FP32 forms have given wrong results now and then: nothing issues them by hand and the compiler is told not to."""
+    assert _holders(r'v_pk_' + r'(add|mul|fma)_f32') == []
+    with open(os.path.join(ROOT, 'pyflac_amd', 'csrc', 'Makefile')) as f:
+        assert '-Xclang -target-feature -Xclang -packed-fp32-ops' in f.read()
+
+
+@pytest.mark.skipif(not os.path.exists(OBJDUMP), reason='needs llvm-objdump')
+def test_the_built_library_holds_no_packed_fp32(tmp_path):
+    """The gfx950 assembly of every code object built here."""
+    shutil.copy(os.path.join(ROOT, 'pyflac_amd', 'libflacgpu.so'), tmp_path / 'lib.so')
+    subprocess.run([OBJDUMP, '--offloading', 'lib.so'], cwd=tmp_path, check=True, capture_output=True)
+    objs = sorted(f for f in os.listdir(tmp_path) if 'gfx950' in f)
+    assert len(objs) >= 10
+    for o in objs:
+        text = subprocess.run([OBJDUMP, '-d', '--no-show-raw-insn', '--mcpu=gfx950', o], cwd=tmp_path, check=True, capture_output=True, text=True).stdout
+        assert 's_endpgm' in text and not re.search('v_pk_' + '(add|mul|fma)_f32', text), o

@@ -5,7 +5,7 @@ import glob, os, re, subprocess, sys, tempfile
 root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 src = os.path.join(root, 'pyflac_amd', 'csrc')
 tag = sys.argv[1] if len(sys.argv) > 1 else 'r03'
-flags = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-ffp-contract=off', '-fno-fast-math', '-I' + os.path.join(root, 'include'), '-I' + src,
+flags = ['--offload-arch=gfx950', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops', '-O3', '-std=c++17', '-fPIC', '-ffp-contract=off', '-fno-fast-math', '-I' + os.path.join(root, 'include'), '-I' + src,
          '--cuda-device-only', '-c', '-o', '/dev/null', '-Rpass-analysis=kernel-resource-usage']
 out = []
 for f in sorted(glob.glob(os.path.join(src, '*.hip'))):

@@ -1,5 +1,5 @@
 // What a LONE wave pays per instruction in dependent chains of the kinds the restore kernel's recurrence is made of (tuning aid;
-// not part of the product).  build: hipcc --offload-arch=gfx950 -O2 -o chainlat chainlat.hip
+// not part of the product).  build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 -o chainlat chainlat.hip
 // 256 workgroups of one wave (one per CU), each runs REPS x a block of one kind; time by wall_clock64 (100 MHz) inside the wave.
 #include <hip/hip_runtime.h>
 #include <stdint.h>

@@ -1,5 +1,5 @@
 // v_mfma_f64_4x4x4_4b_f64 on gfx950: operand layout, rounding order, and cost of a dependent chain (tuning aid; not part of
-// the product).  build: hipcc --offload-arch=gfx950 -O2 -o mfma64 mfma64.hip
+// the product).  build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 -o mfma64 mfma64.hip
 //  1. layout: 64 launches in one kernel -- A one-hot in lane la, B[lane] = lane + 1, C = 0: the output lanes that light up and
 //     their values tell which (A lane, B lane) pairs meet in which output lane.
 //  2. order: random operands with wide exponent spread; the host composes the candidates (fma chain over k ascending /

@@ -1,5 +1,5 @@
 // Issue rate of a few VALU instructions on gfx950 under full occupancy (tuning aid; not part of the product).
-// build: hipcc --offload-arch=gfx950 -O2 -o valurate valurate.hip
+// build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 -o valurate valurate.hip
 // 8192 waves (8 per SIMD), each issues REPS x 16 instructions of one kind on 8 independent accumulators; the kernel time gives
 // cycles per wave-instruction per SIMD at an assumed 2.4 GHz -- the RATIOS between the kinds are what counts.
 #include <hip/hip_runtime.h>
@@ -190,11 +190,6 @@ __global__ void __launch_bounds__(256) k_rate(uint32_t *sink, int reps)
             REP8(S) REP8(S)
 #undef S
         }
-        else if (KIND == 37) {
-#define S(i) asm volatile("v_pk_fma_f32 %0, %1, %1, %0" : "+v"(d[i]) : "v"(e));
-            REP8(S) REP8(S)
-#undef S
-        }
         else if (KIND == 38) {
 #define S(i) asm volatile("v_mul_lo_u32 %0, %1, %0" : "+v"(a[i]) : "v"(b));
             REP8(S) REP8(S)
@@ -310,7 +305,6 @@ int main()
     run<34>("v_xor_b32", sink);
     run<35>("v_ashrrev_i32 v,v", sink);
     run<36>("v_add_u32 sdwa", sink);
-    run<37>("v_pk_fma_f32", sink);
     run<38>("v_mul_lo_u32", sink);
     run<39>("v_mad_u32_u24", sink);
     run<40>("v_lshl_or_b32", sink);
