@@ -66,3 +66,10 @@ def test_the_built_library_holds_no_packed_fp32(tmp_path):
     for o in objs:
         text = subprocess.run([OBJDUMP, '-d', '--no-show-raw-insn', '--mcpu=gfx950', o], cwd=tmp_path, check=True, capture_output=True, text=True).stdout
         assert 's_endpgm' in text and not re.search('v_pk_' + '(add|mul|fma)_f32', text), o
+
+
+def test_no_build_leftover_is_tracked():
+    if not os.path.isdir(os.path.join(ROOT, '.git')):
+        pytest.skip('not a checkout')
+    files = subprocess.run(['git', 'ls-files'], cwd=ROOT, check=True, capture_output=True, text=True).stdout.split('\n')
+    assert [f for f in files if f.endswith(('.tmp', '.o', '.so', '.a', '.pyc'))] == []
