@@ -181,18 +181,19 @@ def committed_pmc(workload, level, nblocks, kernel_id, load=None, build_id=None)
     otherwise `same` is False, `traffic` / `issue_ceiling` stay out of the line and `note` says why.  A round-5 pass carries the id
     of the whole build only and counts for exactly that build (`build_id`).  (`load`: committed_profile, replaceable in tests.)"""
     load = load or committed_profile
-    pmc, pmc_name = {}, None
-    for rnd in ('r06', 'r05', 'r04', 'r03', 'r02'):
-        pmc_name = '%s_pmc.json' % rnd if workload == 'stream16' else '%s_pmc_%s.json' % (rnd, workload)
-        pmc = load(pmc_name) or {}
-        if pmc:
-            break
-    same_shape = pmc.get('workload') == workload and pmc.get('level') == level and pmc.get('blocks') == nblocks
-    if pmc.get('kernel_id'):
-        same_code = pmc.get('kernel_id') == kernel_id
-    else:
-        same_code = bool(pmc.get('build_id')) and build_id is not None and pmc.get('build_id') == build_id
-    same = bool(pmc) and same_shape and same_code
+
+    def counts(p):
+        same_shape = p.get('workload') == workload and p.get('level') == level and p.get('blocks') == nblocks
+        if p.get('kernel_id'):
+            return same_shape and p.get('kernel_id') == kernel_id
+        return same_shape and bool(p.get('build_id')) and build_id is not None and p.get('build_id') == build_id
+
+    names = ['%s_pmc.json' % t if workload == 'stream16' else '%s_pmc_%s.json' % (t, workload)
+             for t in ('r06', 'r05', 'r04', 'r03', 'r02', 'plainsums')]
+    passes = [(load(n) or {}, n) for n in names]
+    # the pass of these kernels; else the first there is, which the note names
+    pmc, pmc_name = next((p for p in passes if p[0] and counts(p[0])), None) or next((p for p in passes if p[0]), ({}, names[-1]))
+    same = bool(pmc) and counts(pmc)
     note = None
     if pmc and not same:
         their = ('kernels %s' % pmc['kernel_id']) if pmc.get('kernel_id') else ('build %s' % pmc.get('build_id', '(no id: before round 5)'))
