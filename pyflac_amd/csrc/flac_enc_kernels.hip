@@ -3,7 +3,8 @@
 // Replaces the per-block hot loop of libFLAC's process_frame_/process_subframes_ that pyFLAC
 // reaches through FLAC__stream_encoder_process_interleaved (reference: pyflac/encoder.py:115;
 // algorithm: SURVEY.md Appendix A, rows L2-L13 of section 8a).  Output frames are bit-exact with
-// libFLAC 1.4.3 for the same settings.
+// libFLAC 1.4.3 for the same settings, except that the fixed predictors' error sums are plain for every block length, which
+// some x86-64 builds of it do not do where (length - 4) mod 4 != 0 (tests/cases.py UNPINNED_FUZZ_SEEDS).
 //
 // Mapping (wave64, block = one wavefront):
 //   * samples are staged once from HBM into LDS (planar int32, two channels at a time);

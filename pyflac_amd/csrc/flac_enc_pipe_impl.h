@@ -27,7 +27,8 @@
 //                               the CRC-16 and writes the frame at its final byte offset in the output stream (this
 //                               replaces the slot -> stream compaction copy of round 1).
 //
-// Bytes are identical to the round-1 kernels and to libFLAC 1.4.3 (tests/test_gpu_encode.py).
+// Bytes are identical to the generic kernel's and, but for the block lengths that flac_enc_kernels.hip names, to libFLAC 1.4.3
+// (tests/test_gpu_encode.py, tests/test_gpu_fixed_sums.py).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>

@@ -91,6 +91,6 @@ def test_unpinned_seeds_are_valid_and_lossless(seed, fuzz_golden):
 
 @pytest.mark.skipif(not os.path.exists('/opt/rocm/lib/llvm/bin/llvm-objdump'), reason='the emulator reads the code objects through llvm-objdump')
 def test_compiled_kernels_against_the_oracle_on_the_emulator():
-    p = subprocess.run([sys.executable, '-m', 'pytest', '-q', '-x', '-p', 'tests.emu.plugin', '-m', 'gpu', 'tests/test_gpu_fixed_sums.py'],
+    p = subprocess.run([sys.executable, '-m', 'pytest', '-q', '-x', '-p', 'tests.emu.plugin', '-m', 'gpu', '-k', 'not recorded_ones', 'tests/test_gpu_fixed_sums.py'],
                        capture_output=True, text=True, timeout=550, cwd=ROOT)
     assert p.returncode == 0 and ' failed' not in p.stdout, (p.stdout[-3000:], p.stderr[-2000:])
